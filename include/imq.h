@@ -287,8 +287,7 @@ int imq_linear_f8(const void* x, int64_t x_row_stride, int x_dtype, int64_t M, i
 
 /* A MoE layer's routed experts: [g | u] = gate_up_e(x_t), h = silu(g) u, out[t] = sum_j w[t, j] down_e(h), e =
  * topk_idx[t, j], every projection as imq_linear_f8, but g and u of exact products, as h is quantized (from its fp32 values)
- * and a sum's error would decide codes. The routed rows are kept in fp32 (few tokens) or in fp16 with a shared exponent per
- * 32 to 128 columns, their weighted sum is taken in fp32.
+ * and a sum's error would decide codes. The routed rows are kept in fp32, and so is their weighted sum.
  *   hidden [T, H] (bf16 / fp16 / fp32), topk_idx [T, k] contiguous (IMQ_DT_I32 / IMQ_DT_I64; ids outside [0, E) count
  *   as expert 0), topk_w [T, k] contiguous (bf16 / fp16 / fp32).
  *   gate_up e4m3 [E, 2 I, H_pad], rows [gate | up]; its scales [E, 2 ceil(I/128), H_pad/128]: gate's blocks, then

@@ -64,13 +64,6 @@ IMQ_DEV float f8_silu_mul(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.f + e) * u;
 }
 
-// Two fp32 values -> packed fp16, round to nearest even.
-IMQ_DEV uint32_t f8_pk_f16(float lo, float hi) {
-  typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
-  const f32x2_t v = {lo, hi};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
-}
-
 // 16x16x128: A lane l = row l % 16, B lane l = column l % 16, 32 of the 128 bytes in lanes l / 16; D lane l holds
 // column l % 16, rows 4 (l / 16) .. + 3.
 IMQ_DEV f32x4_t mfma_f8_16x16x128(i32x8_t a, i32x8_t b, f32x4_t c) {

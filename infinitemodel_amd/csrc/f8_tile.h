@@ -12,7 +12,7 @@
 // MODE 1: the experts' gate_up: rows sorted by expert, tile rows [0, BN/2) gate and [BN/2, BN) up of the same
 //         128 columns of h; the epilogue forms h = silu(g) u in fp32 and quantizes it. Products by the bf16 instruction
 //         (f8_widen), as h's codes hang on them: 4096 tokens of 8 of 64 experts of 2048 x 1024 take 480 us, 370 without.
-// MODE 2: the experts' down: rows sorted by expert, written back in routed order.
+// MODE 2: the experts' down: rows sorted by expert, written back in routed order, in fp32.
 #pragma once
 
 #include "f8_common.h"
@@ -31,8 +31,7 @@ struct F8Tile {
   int M, N, nb;          // nb: blocks of 128 columns
   uint16_t* y;
   int64_t sy;
-  float* ys;             // MODE 2: the factor of routed row m, columns [32 i, ..) of a wave's range, at m * ysr + i
-  int64_t ysr;
+  float* rows;           // MODE 2: routed row m, fp32, at m * sy
   float* part;           // MODE 0, fp32 partials [splits][M][N] when splits > 1
   int splits;
   int mt, nt;            // tiles along M (MODE 0) and N
@@ -90,7 +89,7 @@ IMQ_DEV i32x8_t f8_frag(const uint8_t* tile, int row, int g) {
 // Bytes of a buffer: weight rows, activation rows, a scale per activation row.
 constexpr int f8_stage_bytes(int BN, int BM) { return (BN + BM) * 128 + (BM < 64 ? 64 : BM) * 4; }
 
-// A tile's results. They go through `lds` (the last step's buffer; 16-byte pieces rotated by the row, as the operands'),
+// A tile's results. Those in bf16 and h's codes go through `lds` (the last step's buffer; 16-byte pieces rotated by the row, as the operands'),
 // so that memory sees whole rows of the tile: a lane holds 4 columns of one row, and storing those 8 bytes at a time cost
 // as much as 30 steps. Waits for the wave's loads before its first store.
 template <int BN, int BM, int WN, int WM, int MODE, typename ACC>
@@ -117,7 +116,21 @@ IMQ_DEV void f8_epilogue(const F8Tile& a, int m0, int mend, int n0, int split, u
       return;
     }
   }
-  if constexpr (MODE != 1) {
+  if constexpr (MODE == 2) {
+    // A routed row stays fp32 until the combine has summed its token's: a column may be as far below its neighbours as it
+    // likes, and one that is not finite spoils no other. Straight from the registers: a lane's 4 columns are 16 bytes, a
+    // row's four lane groups 64 on end.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < IM; ++j) {
+      const int m = m0 + wm * TM + j * 16 + c;
+      if (m >= mend) continue;
+      float* y = a.rows + (int64_t)a.perm[m] * a.sy + n0 + wn * TN + 4 * g;
+#pragma unroll
+      for (int i = 0; i < IN; ++i)
+        if (n0 + wn * TN + i * 16 + 4 * g < a.N) *(f32x4_t*)(y + i * 16) = acc[i][j];     // the stride is whole fours, past N slack
+    }
+  } else if constexpr (MODE == 0) {
     constexpr int PC = BN / 8;                           // pieces of 8 columns a row
     // the buffer holds BM / PASSES rows at a time
     constexpr int PASSES = BM * BN * 2 > (BN + BM) * 128 ? 2 : 1, ROWS = BM / PASSES;
@@ -131,42 +144,11 @@ IMQ_DEV void f8_epilogue(const F8Tile& a, int m0, int mend, int n0, int split, u
 #pragma unroll
         for (int j = 0; j < IM; ++j) {
           const int row = wm * TM + j * 16 + c;
-          float down = 1.f;
-          if constexpr (MODE == 2) {
-            // a routed row is kept between the launches as fp16 times a power of two per TN columns, that of their
-            // largest magnitude: 11 bits for the values that matter to the sum (bf16's 8 showed in the result, fp32
-            // would double the 2 x 134 MB that 4096 tokens of 8 experts move)
-            uint32_t mx = 0;
-#pragma unroll
-            for (int i = 0; i < IN; ++i)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint32_t bits = __float_as_uint(acc[i][j][r]) & 0x7fffffffu;
-                mx = bits > mx ? bits : mx;
-              }
-#pragma unroll
-            for (int o = 16; o < 64; o <<= 1) {
-              const uint32_t q = (uint32_t)__shfl_xor((int)mx, o, 64);
-              mx = q > mx ? q : mx;
-            }
-            uint32_t ex = mx >> 23;
-            ex = ex < 1 ? 1 : ex > 253 ? 253 : ex;       // the power and its reciprocal are normal floats
-            down = __uint_as_float((254 - ex) << 23);
-            if (g == 0 && m0 + row < mend && n0 + wn * TN < a.N)
-              a.ys[(int64_t)a.perm[m0 + row] * a.ysr + (n0 + wn * TN) / 32] = __uint_as_float(ex << 23);
-          }
           const int at = row - s * ROWS;
 #pragma unroll
           for (int i = 0; i < IN; ++i) {
             const int piece = (wn * TN + i * 16) / 8 + (g >> 1);
-            u32x2_t w;
-            if constexpr (MODE == 2) {
-#pragma unroll
-              for (int q = 0; q < 2; ++q)
-                w[q] = f8_pk_f16(acc[i][j][2 * q] * down, acc[i][j][2 * q + 1] * down);
-            } else {
-              w = u32x2_t{cvt_pk_bf16(acc[i][j][0], acc[i][j][1]), cvt_pk_bf16(acc[i][j][2], acc[i][j][3])};
-            }
+            const u32x2_t w = {cvt_pk_bf16(acc[i][j][0], acc[i][j][1]), cvt_pk_bf16(acc[i][j][2], acc[i][j][3])};
             *(u32x2_t*)(lds + at * (BN * 2) + ((piece ^ (at & (PC - 1))) << 4) + 8 * (g & 1)) = w;
           }
         }
@@ -175,11 +157,12 @@ IMQ_DEV void f8_epilogue(const F8Tile& a, int m0, int mend, int n0, int split, u
       lds_barrier();
 #pragma unroll 4
       for (int id = tid; id < ROWS * PC; id += 64 * W) {
-        const int at = id / PC, piece = id % PC, n = n0 + piece * 8, m = m0 + s * ROWS + at;
+        const int at = id / PC, piece = id % PC, n = n0 + piece * 8;
+        const int64_t m = m0 + s * ROWS + at;
         if (m >= mend || n >= a.N) continue;
         const u32x4_t v = *(const u32x4_t*)(lds + at * (BN * 2) + ((piece ^ (at & (PC - 1))) << 4));
-        uint16_t* y = a.y + (MODE == 2 ? (int64_t)a.perm[m] : (int64_t)m) * a.sy + n;
-        if (MODE == 2 || (vec && n + 8 <= a.N)) {        // MODE 2: the stride is a multiple of 8, past N it is slack
+        uint16_t* y = a.y + m * a.sy + n;
+        if (vec && n + 8 <= a.N) {
           *(u32x4_t*)y = v;
         } else {
 #pragma unroll

@@ -133,11 +133,10 @@ __global__ __launch_bounds__(256) void f8_place_kernel(const void* __restrict__ 
   f8_place(c, E, bm, lds, blockIdx.x == 0, perm, tiles);
 }
 
-// out[t] = sum over j, in order, of w[t, j] y[t k + j] in fp32: 8 columns a thread. y: fp16 times a factor per 2^sh
-// columns (f8_tile.h, MODE 2).
-__global__ __launch_bounds__(256) void f8_combine_kernel(const uint16_t* __restrict__ y, int64_t sy, const float* __restrict__ ys,
-                                                         int64_t ysr, int sh, const void* __restrict__ w, int wdt, int k, int64_t H,
-                                                         FastDiv per, int64_t total, uint16_t* __restrict__ out, int64_t so) {
+// out[t] = sum over j, in order, of w[t, j] y[t k + j] in fp32: 8 columns a thread. y: fp32, rows padded to whole eights.
+__global__ __launch_bounds__(256) void f8_combine_kernel(const float* __restrict__ y, int64_t sy, const void* __restrict__ w, int wdt,
+                                                         int k, int64_t H, FastDiv per, int64_t total, uint16_t* __restrict__ out,
+                                                         int64_t so) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (id >= total) return;
   const int64_t t = div_fast((uint32_t)id, per), n = (id - t * per.d) * 8;
@@ -145,13 +144,12 @@ __global__ __launch_bounds__(256) void f8_combine_kernel(const uint16_t* __restr
 #pragma unroll 4
   for (int j = 0; j < k; ++j) {
     const int64_t b = t * k + j;
-    const float c = f8_weight_at(w, wdt, b), s = ys[b * ysr + ((n >> sh) << sh) / 32];
-    const u32x4_t d = *(const u32x4_t*)(y + b * sy + n);
+    const float c = f8_weight_at(w, wdt, b);
+    const f32x4_t d0 = *(const f32x4_t*)(y + b * sy + n), d1 = *(const f32x4_t*)(y + b * sy + n + 4);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t p = d[i];
-      v[2 * i] = fmaf(c, f16_bits_to_f32(p & 0xffffu) * s, v[2 * i]);
-      v[2 * i + 1] = fmaf(c, f16_bits_to_f32(p >> 16) * s, v[2 * i + 1]);
+      v[i] = fmaf(c, d0[i], v[i]);
+      v[4 + i] = fmaf(c, d1[i], v[4 + i]);
     }
   }
   uint16_t* o = out + t * so + n;
@@ -189,7 +187,7 @@ Plan plan_of(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, const DevInf
 }
 
 struct Ws {
-  int64_t xq, xs, hq, hs, y, ys, ysr, counts, perm, tiles, total, sy;
+  int64_t xq, xs, hq, hs, y, counts, perm, tiles, total, sy;
 };
 
 Ws ws_of(const Plan& p, int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
@@ -200,14 +198,12 @@ Ws ws_of(const Plan& p, int64_t T, int64_t k, int64_t E, int64_t H, int64_t I) {
     return w;
   }
   w.sy = (H + 7) / 8 * 8;
-  w.ysr = hb * 4;
   w.xq = 0;
   w.xs = w.xq + up256(T * hb * F8_BLOCK);
   w.hq = w.xs + up256(T * hb * 4);
   w.hs = w.hq + up256(B * ib * F8_BLOCK);
   w.y = w.hs + up256(B * ib * 4);
-  w.ys = w.y + up256(B * w.sy * 2);
-  w.counts = w.ys + up256(B * w.ysr * 4);
+  w.counts = w.y + up256(B * w.sy * 4);
   w.perm = w.counts + up256(imq_cdiv(B, kChunk) * E * 4);
   w.tiles = w.perm + up256(B * 4);
   w.total = w.tiles + up256((1 + 3 * (B / p.bm + (B < E ? B : E))) * 4);
@@ -394,18 +390,15 @@ extern "C" int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int 
   d.splits = 1;
   d.tiles = tl;
   d.perm = perm;
-  d.y = (uint16_t*)(ws + L.y);
+  d.rows = (float*)(ws + L.y);
   d.sy = L.sy;
-  d.ys = (float*)(ws + L.ys);
-  d.ysr = L.ysr;
   d.nt = (int)imq_cdiv(H, bm == 192 ? 256 : 128);
   rc = bm == 192 ? go<256, 192, 2, 4, 2, 2>(d, tiles, dev.cus, st) : bm == 128 ? go<128, 128, 2, 2, 2, 2>(d, tiles, dev.cus, st)
        : bm == 64 ? go<128, 64, 4, 1, 3, 2>(d, tiles, dev.cus, st) : go<128, 32, 4, 1, 3, 2>(d, tiles, dev.cus, st);
   if (rc != IMQ_OK) return rc;
-  const int sh = bm == 192 ? 7 : bm == 128 ? 6 : 5;      // log2 of the columns of a wave of the down kernel
   const int64_t cols = imq_cdiv(H, 8), total = T * cols;
   f8_combine_kernel<<<dim3((unsigned)imq_cdiv(total, 256)), dim3(256), 0, st>>>(
-      d.y, d.sy, d.ys, d.ysr, sh, topk_w, w_dtype, (int)top_k, H, fast_div((uint32_t)cols), total, (uint16_t*)out, out_row_stride);
+      d.rows, d.sy, topk_w, w_dtype, (int)top_k, H, fast_div((uint32_t)cols), total, (uint16_t*)out, out_row_stride);
   IMQ_LAUNCH_CHECK();
   return IMQ_OK;
 }

@@ -83,7 +83,7 @@ def experts(xv, ids, w, gu, dn, H, I):
     """(out, bound) of a MoE layer's experts on quantized rows xv [T, H_pad]; gu / dn = (codes [E, .., K_pad], scales).
     Gate and up are sums of exact products. The bound follows the sums' errors through silu, through the second
     quantization (a value of h that close to a rounding border may take either code) and the down projection; the routed
-    rows (fp16 with a shared exponent at the least) and the result are rounded."""
+    rows are summed in fp32 and the result is rounded."""
     (gq, gs), (dq, ds) = gu, dn
     T, k = ids.shape
     ib = blocks(I)
@@ -112,8 +112,6 @@ def experts(xv, ids, w, gu, dn, H, I):
         width = np.maximum(np.abs(hi * sv - np.abs(hv)), np.abs(lo * sv - np.abs(hv))) + np.maximum(hi, np.abs(hv) / sv) * es
         y = hv @ wd.T
         ey = width @ np.abs(wd).T + sum_slack(hv.shape[1]) * ((np.abs(hv) + width) @ np.abs(wd).T) + cut_slack(np.abs(hv) + width, wd)
-        # fp16 times the power of two of the largest magnitude of its columns: half a step, 2^-25 of that power at least
-        ey = ey + 2.0 ** -11 * (np.abs(y) + ey) + 2.0 ** -24 * (np.abs(y) + ey).max(axis=1, keepdims=True)
         c = w[t, j].astype(np.float64)[:, None]
         np.add.at(out, t, c * y)
         np.add.at(tol, t, np.abs(c) * ey + k * 2.0 ** -23 * np.abs(c * y))

@@ -1,0 +1,91 @@
+"""The fp8 operators on values where a form may go wrong alone: codes that are NaN, columns far below their neighbours, values
+on the border between two codes, gates at the ends of fp32. Each case in every form of the experts: the direct one and the row
+tiles of 32, 64, 128 and 192."""
+import numpy as np
+import pytest
+
+from oracle import f8 as of
+
+pytestmark = pytest.mark.gpu
+# tokens of one of four experts each: the direct form, then 20, 40, 150 and 250 mean rows an expert
+TOKENS = (3, 80, 160, 600, 1000)
+
+
+def _codes_dev(dev, q):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(q)).to(dev).view(torch.float8_e4m3fn)
+
+
+def _layer(dev, E, H, I, seed):
+    """Random experts: what the oracle takes and what the call takes."""
+    import torch
+    r = np.random.default_rng(seed)
+    hb, ib = of.blocks(H), of.blocks(I)
+    gq = of.codes_of(np.clip(r.standard_normal((E, 2 * I, hb * 128)) * 100, -448, 448))
+    dq = of.codes_of(np.clip(r.standard_normal((E, H, ib * 128)) * 100, -448, 448))
+    gq[..., H:], dq[..., I:] = 0, 0
+    gs, ds = (r.uniform(1e-4, 3e-4, s).astype(np.float32) for s in ((E, 2 * ib, hb), (E, hb, ib)))
+    return gq, gs, dq, ds, [torch.from_numpy(s).to(dev) for s in (gs, ds)]
+
+
+def _routing(dev, T, E, k, seed):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    w, ids = torch.topk(torch.softmax(torch.randn(T, E, generator=g), -1), k, -1)
+    return w.to(dev), ids.to(dev)
+
+
+def _np(t):
+    import torch
+    return t.detach().to(torch.float64).cpu().numpy()
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_nan_codes_spoil_what_they_are_part_of(dev, T):
+    """A NaN code of a down weight makes its column NaN for the tokens that its expert serves, one of a gate or up weight the
+    whole of those tokens; every other output is what it is without them."""
+    import torch
+    from infinitemodel_amd import ops
+    E, H, I, k = 4, 300, 256, 1
+    gq, gs, dq, ds, (gst, dst) = _layer(dev, E, H, I, seed=T)
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16).to(dev)
+    w, ids = _routing(dev, T, E, k, seed=T)
+    want, tol = of.experts(of.dequantize(*of.quantize(_np(x))), ids.cpu().numpy(), w.cpu().numpy(), (gq, gs), (dq, ds), H, I)
+    mine = _np(ids)[:, 0].astype(int)
+    e = int(mine[0])
+    for place in ("down", "gate", "up"):
+        g, d = gq.copy(), dq.copy()
+        bad = np.zeros((T, H), dtype=bool)
+        if place == "down":
+            d[e, 1, 5], d[e, 130, 255], d[e, 299, 0] = 0x7f, 0xff, 0x7f
+            bad[:, [1, 130, 299]] = (mine == e)[:, None]
+        else:
+            g[e, 7 if place == "gate" else I + 200, 3] = 0x7f
+            bad[mine == e] = True
+        out = _np(ops.moe_experts_f8(x, ids, w, (_codes_dev(dev, g), gst, H), (_codes_dev(dev, d), dst, I)))
+        np.testing.assert_array_equal(np.isnan(out), bad)
+        assert (np.abs(out - want) <= tol)[~bad].all(), place
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_columns_far_below_their_neighbours(dev, T):
+    """A column 2^-36 of the one beside it comes out as exact as that one: h holds 448 and 2^-9, and each output is one product of
+    a code of down with one of them."""
+    import torch
+    from infinitemodel_amd import ops
+    E, H, I = 4, 128, 128
+    one, gate = of.codes_of(np.array([1.0, 64.0]))
+    gq, dq = np.zeros((E, 2 * I, 128), np.uint8), np.zeros((E, H, 128), np.uint8)
+    gq[:, :I, 1] = gate                                       # g = 64 at every column: silu(64) is 64 in fp32
+    gq[:, I, 1], gq[:, I + 1, 1] = of.codes_of(np.array([448.0, 2.0 ** -9]))
+    dq[:, 0, 0] = of.codes_of(np.array(448.0))
+    dq[:, 1:, 1] = np.arange(1, H)                            # every magnitude from 2^-9 on
+    s = torch.ones(E, 2, 1, device=dev), torch.ones(E, 1, 1, device=dev)
+    x = torch.zeros(T, H)
+    x[:, 0], x[:, 1] = 448.0, 1.0                             # scale 1
+    ids = (torch.arange(T) % E)[:, None].to(dev)
+    dq[:, 127, 1] = one
+    out = ops.moe_experts_f8(x.to(dev), ids, torch.ones(T, 1, device=dev), (_codes_dev(dev, gq), s[0], H), (_codes_dev(dev, dq), s[1], I))
+    want = 64 * of.values_of(dq[0, :, 1]) * 2.0 ** -9
+    want[0] = 64 * 448.0 * 448.0
+    np.testing.assert_array_equal(_np(out), np.tile(want, (T, 1)))
