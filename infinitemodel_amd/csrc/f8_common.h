@@ -45,14 +45,6 @@ IMQ_DEV uint32_t f8_codes4(const float* v, float s, float r) {
   return s != s ? 0u : (uint32_t)w;
 }
 
-// The same by the reciprocal, where x is an fp32 result that is itself off by a step or more: the quotient is off by
-// at most two, so a value that close to a border may go to either side of it, as it may by its own error.
-IMQ_DEV uint32_t f8_codes4_near(const float* v, float s, float r) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * r, v[1] * r, 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * r, v[3] * r, w, true);
-  return s != s ? 0u : (uint32_t)w;
-}
-
 // silu(g) u to a few steps of fp32: e^-g by the hardware's exponential of t = -g / ln 2, whose rounding (and that of 1 / ln 2)
 // is carried on in `lo`; the reciprocal is off by one step. Half the operations of expf and a division, which
 // were half of the gate_up tile's epilogue. t is cut at 126, below which silu is 0 in any sum.

@@ -215,7 +215,7 @@ IMQ_DEV void f8_epilogue(const F8Tile& a, int m0, int mend, int n0, int split, u
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = acc[i][j][q];
         const int piece = (wn * (TN / 2)) / 16 + i;
-        *(uint32_t*)(lds + row * 128 + (f8_slot(row, piece) << 4) + 4 * g) = f8_codes4_near(v, s, rs);
+        *(uint32_t*)(lds + row * 128 + (f8_slot(row, piece) << 4) + 4 * g) = f8_codes4(v, s, rs);
       }
       if (wn == 0 && g == 0 && m < mend) a.hs[(int64_t)(n0 / 128) * a.hsb + m] = s;
     }

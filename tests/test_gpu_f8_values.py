@@ -89,3 +89,36 @@ def test_columns_far_below_their_neighbours(dev, T):
     want = 64 * of.values_of(dq[0, :, 1]) * 2.0 ** -9
     want[0] = 64 * 448.0 * 448.0
     np.testing.assert_array_equal(_np(out), np.tile(want, (T, 1)))
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_h_on_the_border_of_two_codes(dev, T):
+    """h's codes are e4m3 of the exact quotient, in every form: values halfway between two codes, at scales whose rounded
+    reciprocal would put some of them on the other side."""
+    import torch
+    from infinitemodel_amd import ops
+    E, H, I = 4, 128, 128
+    mids = of.MIDS[(of.MIDS >= 17) & (of.MIDS == np.round(of.MIDS))]
+    gq, dq, want = np.zeros((E, 2 * I, 128), np.uint8), np.zeros((E, H, 128), np.uint8), np.zeros((E, H))
+    gq[:, :I, 1] = of.codes_of(np.array(64.0))               # g = 64: silu(g) u is 64 u in fp32
+    dq[:, np.arange(I), np.arange(I)] = of.codes_of(np.array(1.0))
+    for e, j in enumerate((7, 15, 61, 126)):                  # the block's scale is 64 j
+        u = np.zeros(I, dtype=np.int64)
+        u[0], u[1:1 + len(mids)] = 448 * j, mids * j
+        digits = [u >> 12 & 15, u >> 8 & 15, u >> 4 & 15, u & 15]          # times 4096, 256, 16, 1
+        for col, d in enumerate(digits):
+            gq[e, I:, 2 + col] = of.codes_of(d * (16.0 if col == 0 else 1.0))
+        h = 64.0 * u
+        s = np.float32(64 * j)
+        codes = of.codes_of(h / np.float64(s))
+        assert (codes != of.codes_of((h.astype(np.float32) * (np.float32(1) / s)).astype(np.float64))).any()
+        want[e] = of.values_of(codes) * 64 * j
+    s = torch.ones(E, 2, 1, device=dev), torch.ones(E, 1, 1, device=dev)
+    x = torch.zeros(T, H)
+    x[:, 0] = 448.0                                           # scale 1
+    x[:, 1:6] = torch.tensor([1.0, 256.0, 256.0, 16.0, 1.0])
+    ids = torch.arange(T) % E
+    out = ops.moe_experts_f8(x.to(dev), ids[:, None].to(dev), torch.ones(T, 1, device=dev), (_codes_dev(dev, gq), s[0], H),
+                             (_codes_dev(dev, dq), s[1], I))
+    w = want[ids.numpy()]
+    assert (np.abs(_np(out) - w) <= 2.0 ** -8 * w).all()       # bf16's rounding; the next code is 2^-4 away
