@@ -45,15 +45,18 @@ IMQ_DEV uint32_t f8_codes4(const float* v, float s, float r) {
   return s != s ? 0u : (uint32_t)w;
 }
 
-// silu(g) u to a few steps of fp32: e^-g by the hardware's exponential of t = -g / ln 2, whose rounding (and that of 1 / ln 2)
+// silu(g) u = g u / (1 + e^-g) to a few steps of fp32, from e = e^-|g|, which cannot overflow: g / (1 + e) where g is positive, g e /
+// (1 + e) where it is negative. e by the hardware's exponential of t = -|g| / ln 2, whose rounding (and that of 1 / ln 2)
 // is carried on in `lo`; the reciprocal is off by one step. Half the operations of expf and a division, which
-// were half of the gate_up tile's epilogue. t is cut at 126, below which silu is 0 in any sum.
+// were half of the gate_up tile's epilogue. |g| is cut at 87, so e is a normal number; silu of less than -87, below 2^-119
+// in magnitude, is taken as 0. NaN and -inf (infinity times 0) give NaN.
 IMQ_DEV float f8_silu_mul(float g, float u) {
-  const float t = fminf(g * -1.44269504f, 126.f);
-  const float lo = fmaf(g, -1.92596302e-8f, fmaf(g, -1.44269504f, -t));
+  const float a = fabsf(g), m = fminf(a, 87.f), t = m * -1.44269504f;
+  const float lo = fmaf(m, -1.92596302e-8f, fmaf(m, -1.44269504f, -t));
   float e = __builtin_amdgcn_exp2f(t);
-  e = fmaf(e, t < 126.f ? lo * 0.693147181f : 0.f, e);
-  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+  e = fmaf(e, lo * 0.693147181f, e);
+  const float f = g >= 0.f ? 1.f : a > 87.f ? 0.f : e;
+  return g * f * __builtin_amdgcn_rcpf(1.f + e) * u;
 }
 
 // 16x16x128: A lane l = row l % 16, B lane l = column l % 16, 32 of the 128 bytes in lanes l / 16; D lane l holds

@@ -122,3 +122,38 @@ def test_h_on_the_border_of_two_codes(dev, T):
                              (_codes_dev(dev, dq), s[1], I))
     w = want[ids.numpy()]
     assert (np.abs(_np(out) - w) <= 2.0 ** -8 * w).all()       # bf16's rounding; the next code is 2^-4 away
+
+
+@pytest.mark.parametrize("T", TOKENS)
+def test_gates_at_the_ends_of_fp32(dev, T):
+    """silu of gates up to 3e38 of either sign, beside an ordinary one in the same block of h: g itself or 0, and never NaN."""
+    import torch
+    from infinitemodel_amd import ops
+    E, H, I = 4, 256, 128
+    sizes = [2.0 ** 119, 2.0 ** 60, 1.0, 0.125]               # of each expert's gate, in the first 128 columns
+    codes = np.array([448.0, 256.0, 1.0, 2.0 ** -9])
+    gq, dq = np.zeros((E, 2 * I, 256), np.uint8), np.zeros((E, H, 128), np.uint8)
+    gq[:, :4, 1] = of.codes_of(codes)
+    gq[:, 4, 129] = of.codes_of(np.array(64.0))
+    gq[:, I:I + 4, 129] = of.codes_of(np.array(2.0 ** -9))
+    gq[:, I + 4, 129] = of.codes_of(np.array(1.0))
+    dq[:, np.arange(5), np.arange(5)] = of.codes_of(np.array(1.0))
+    gs = np.ones((E, 2, 2), np.float32)
+    gs[:, 0, 0] = sizes
+    x = torch.zeros(T, H)
+    x[:, [0, 128]] = 448.0                                    # scale 1
+    sign = torch.where(torch.arange(T) % 8 < 4, 1.0, -1.0) if T > 4 else torch.tensor([1.0, -1.0, 1.0])
+    x[:, 1], x[:, 129] = sign, 1.0
+    ids = torch.arange(T) % E if T > 4 else torch.zeros(T, dtype=torch.int64)
+    out = _np(ops.moe_experts_f8(x.to(dev), ids[:, None].to(dev), torch.ones(T, 1, device=dev),
+                                 (_codes_dev(dev, gq), torch.from_numpy(gs).to(dev), H), (_codes_dev(dev, dq), torch.ones(E, 2, 1, device=dev), I)))
+    g = sign.double().numpy()[:, None] * np.array(sizes)[ids.numpy()][:, None] * codes
+    h = np.zeros((T, I))
+    h[:, :4] = np.where(g < -700, 0.0, g / (1 + np.exp(-np.maximum(g, -700)))) * 2.0 ** -9
+    h[:, 4] = 64.0
+    q, s = of.quantize(h)
+    near = np.abs(h / s.astype(np.float64))[:, :5, None] / of.MIDS - 1
+    assert np.abs(near).min() > 1e-4                          # no value where fp32's errors would choose the code
+    want = of.dequantize(q, s)[:, :5]
+    assert (np.abs(out[:, :5] - want) <= 2.0 ** -8 * np.abs(want)).all()
+    assert not out[:, 5:].any()
