@@ -294,7 +294,9 @@ int imq_linear_f8(const void* x, int64_t x_row_stride, int x_dtype, int64_t M, i
  *   up's (each projection is blocked by itself). down e4m3 [E, H, I_pad], scales [E, ceil(H/128), I_pad/128].
  *   Scales have unit block stride. out bf16 [T, H]. E <= 4096; T H_pad, T k I_pad and a stack's bytes per expert below 2^31
  *   (else IMQ_ERR_UNSUPPORTED).
- *   workspace: imq_moe_f8_workspace_bytes bytes (-1 for sizes that are refused), as imq_linear_f8's. */
+ *   workspace: imq_moe_f8_workspace_bytes bytes (-1 for sizes that are refused), as imq_linear_f8's.
+ * Both products refuse what they refuse before they look at the workspace: without one, IMQ_ERR_SCRATCH says that nothing else is
+ * wrong. */
 int64_t imq_moe_f8_workspace_bytes(int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I);
 int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int h_dtype, int64_t T, int64_t H, int64_t top_k,
                        const void* topk_idx, int idx_dtype, const void* topk_w, int w_dtype, int64_t E, const void* gu_q,

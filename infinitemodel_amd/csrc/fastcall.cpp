@@ -312,6 +312,14 @@ bool f8_rows(const at::Tensor& q, int64_t dim) {
   return true;
 }
 
+// Whether `need` bytes of workspace are there already. Where they are not, an fp8 call is first put without any, which
+// launches nothing (IMQ_ERR_SCRATCH if nothing else is wrong): what it refuses must not take memory for ever.
+bool f8_held(int dev, void* stream, int64_t need) {
+  if (need <= 0) return true;
+  const auto at = scratches.find({dev, stream});
+  return at != scratches.end() && at->second.bytes >= need;
+}
+
 PyObject* pair(at::Tensor&& a, at::Tensor&& b) {
   PyObject* pa = THPVariable_Wrap(std::move(a));
   PyObject* pb = pa ? THPVariable_Wrap(std::move(b)) : nullptr;
@@ -394,18 +402,23 @@ PyObject* linear_f8_call(PyObject* const* args, Py_ssize_t n) {
   if (given && (xs->scalar_type() != at::kFloat || xs->dim() != 2 || xs->size(0) != M || xs->size(1) != nb)) Py_RETURN_NONE;
   const int code = given ? IMQ_DT_F8 : dtype_code(x->scalar_type());
   void* stream = (void*)c10::hip::getCurrentHIPStream(dev).stream();
-  Scratch ws;
-  if (!scratch(dev, stream, api.f8_ws(M, N, Kp, code), &ws)) return nullptr;
   at::Tensor y = at::empty({M, N}, x->options().requires_grad(false).dtype(at::kBFloat16));
   void *xp = x->data_ptr(), *qp = q->data_ptr(), *yp = y.data_ptr();
   const float *sp = s->data_ptr<float>(), *xsp = given ? xs->data_ptr<float>() : nullptr;
   const int64_t sx = x->stride(0), x0 = given ? xs->stride(0) : 0, x1 = given ? xs->stride(1) : 0, sq = q->stride(0),
                 s0 = s->stride(0), s1 = s->stride(1);
+  auto go = [&](int64_t p, int64_t b) {
+    return api.f8(xp, sx, code, M, K, xsp, x0, x1, qp, sq, sp, s0, s1, N, Kp, yp, N, (void*)p, b, stream);
+  };
+  const int64_t need = api.f8_ws(M, N, Kp, code);
+  if (!f8_held(dev, stream, need) && go(0, 0) != IMQ_ERR_SCRATCH) Py_RETURN_NONE;
+  Scratch ws;
+  if (!scratch(dev, stream, need, &ws)) return nullptr;
   int rc;
   Held held;
   if (!held.take(ws)) return nullptr;
   Py_BEGIN_ALLOW_THREADS;
-  rc = api.f8(xp, sx, code, M, K, xsp, x0, x1, qp, sq, sp, s0, s1, N, Kp, yp, N, (void*)ws.ptr, ws.bytes, stream);
+  rc = go(ws.ptr, ws.bytes);
   Py_END_ALLOW_THREADS;
   if (rc != IMQ_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(y));
@@ -448,8 +461,6 @@ PyObject* moe_f8_call(PyObject* const* args, Py_ssize_t n) {
   const int wdt = dtype_code(w->scalar_type());
   if (k < 1 || idx->size(0) != T || wdt < 0 || !w->is_contiguous() || w->sizes() != idx->sizes()) Py_RETURN_NONE;
   void* stream = (void*)c10::hip::getCurrentHIPStream(dev).stream();
-  Scratch ws;
-  if (!scratch(dev, stream, api.moe_f8_ws(T, k, E, H, I), &ws)) return nullptr;
   at::Tensor out = at::empty({T, H}, x->options().requires_grad(false).dtype(at::kBFloat16));
   void *xp = x->data_ptr(), *ip = idx->data_ptr(), *wp = w->data_ptr(), *gp = q[0]->data_ptr(), *dp = q[1]->data_ptr(),
        *op = out.data_ptr();
@@ -457,12 +468,19 @@ PyObject* moe_f8_call(PyObject* const* args, Py_ssize_t n) {
   const int64_t sx = x->stride(0), g0 = q[0]->stride(0), g1 = q[0]->stride(1), d0 = q[1]->stride(0), d1 = q[1]->stride(1);
   const int64_t gs0 = s[0]->stride(0), gs1 = s[0]->stride(1), ds0 = s[1]->stride(0), ds1 = s[1]->stride(1);
   const int xdt = dtype_code(x->scalar_type()), idt = idx->scalar_type() == at::kLong ? IMQ_DT_I64 : IMQ_DT_I32;
+  auto go = [&](int64_t p, int64_t b) {
+    return api.moe_f8(xp, sx, xdt, T, H, k, ip, idt, wp, wdt, E, gp, g0, g1, gs, gs0, gs1, I, dp, d0, d1, ds, ds0, ds1, op, H,
+                      (void*)p, b, stream);
+  };
+  const int64_t need = api.moe_f8_ws(T, k, E, H, I);
+  if (!f8_held(dev, stream, need) && go(0, 0) != IMQ_ERR_SCRATCH) Py_RETURN_NONE;
+  Scratch ws;
+  if (!scratch(dev, stream, need, &ws)) return nullptr;
   int rc;
   Held held;
   if (!held.take(ws)) return nullptr;
   Py_BEGIN_ALLOW_THREADS;
-  rc = api.moe_f8(xp, sx, xdt, T, H, k, ip, idt, wp, wdt, E, gp, g0, g1, gs, gs0, gs1, I, dp, d0, d1, ds, ds0, ds1, op, H,
-                  (void*)ws.ptr, ws.bytes, stream);
+  rc = go(ws.ptr, ws.bytes);
   Py_END_ALLOW_THREADS;
   if (rc != IMQ_OK) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(out));

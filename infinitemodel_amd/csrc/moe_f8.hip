@@ -233,12 +233,24 @@ int go_gemv(const F8Gemv& a, int64_t grid, int64_t gy, int64_t rows, hipStream_t
 bool float_type(int dt) { return dt == IMQ_DT_BF16 || dt == IMQ_DT_FP16 || dt == IMQ_DT_FP32; }
 constexpr int64_t kMaxExperts = 4096;
 
+// Sizes whose offsets the kernels can hold in 32 bits; each limit by division, so that no product of sizes overflows.
+bool sizes_fit(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, const DevInfo& dev) {
+  const int64_t lim = 0x7fffffff;
+  if (E > kMaxExperts || k > lim || T > lim / k || H > lim || I > lim / 2) return false;
+  const int64_t hp = imq_cdiv(H, F8_BLOCK) * F8_BLOCK, ip = imq_cdiv(I, F8_BLOCK) * F8_BLOCK, B = T * k;
+  if (T > lim / hp || B > lim / ip || 2 * I > lim / hp || H > lim / ip) return false;
+  const Plan p = plan_of(T, k, E, H, I, dev);
+  const int64_t tiles = B / p.bm + (B < E ? B : E);
+  return p.direct || (tiles <= lim / imq_cdiv(H, F8_BLOCK) / 8 && tiles <= lim / imq_cdiv(I, F8_BLOCK) / 8);
+}
+
 }  // namespace
 
 extern "C" int64_t imq_moe_f8_workspace_bytes(int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I) {
-  const int64_t lim = 0x7fffffff;
-  if (T < 0 || top_k < 1 || E < 1 || H < 1 || I < 1 || E > kMaxExperts || top_k > lim || T > lim / top_k || H > lim || I > lim) return -1;
-  return T == 0 ? 0 : ws_of(plan_of(T, top_k, E, H, I, device_info()), T, top_k, E, H, I).total;
+  if (T < 0 || top_k < 1 || E < 1 || H < 1 || I < 1) return -1;
+  if (T == 0) return 0;
+  const DevInfo dev = device_info();
+  return sizes_fit(T, top_k, E, H, I, dev) ? ws_of(plan_of(T, top_k, E, H, I, dev), T, top_k, E, H, I).total : -1;
 }
 
 extern "C" int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int h_dtype, int64_t T, int64_t H, int64_t top_k,
@@ -261,11 +273,9 @@ extern "C" int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int 
       (dn_q_stride_e & 15) || ((uintptr_t)gu_s & 3) || ((uintptr_t)dn_s & 3) || ((uintptr_t)out & 1) || ((uintptr_t)workspace & 15))
     return IMQ_ERR_ALIGN;
   const int64_t lim = 0x7fffffff;
-  if (E > kMaxExperts || top_k > lim || T > lim / top_k || H > lim || I > lim / 2 || T > lim / hp || T * top_k > lim / ip ||
-      2 * I > lim / gu_q_row_stride || H > lim / dn_q_row_stride)
-    return IMQ_ERR_UNSUPPORTED;
-  const int64_t B = T * top_k;
   const DevInfo dev = device_info();
+  if (!sizes_fit(T, top_k, E, H, I, dev) || 2 * I > lim / gu_q_row_stride || H > lim / dn_q_row_stride) return IMQ_ERR_UNSUPPORTED;
+  const int64_t B = T * top_k;
   const Plan p = plan_of(T, top_k, E, H, I, dev);
   const Ws L = ws_of(p, T, top_k, E, H, I);
   if (!workspace || workspace_bytes < L.total) return IMQ_ERR_SCRATCH;
@@ -326,7 +336,6 @@ extern "C" int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int 
   }
   const int bm = p.bm;
   const int64_t tiles = B / bm + (B < E ? B : E), blocks = T * hb, chunks = imq_cdiv(B, kChunk);
-  if (tiles > lim / imq_cdiv(H, 128) / 8 || tiles > lim / ib / 8) return IMQ_ERR_UNSUPPORTED;
   uint8_t *xq = (uint8_t*)(ws + L.xq), *hq = (uint8_t*)(ws + L.hq);
   float *xs = (float*)(ws + L.xs), *hs = (float*)(ws + L.hs);
   int32_t *counts = (int32_t*)(ws + L.counts), *perm = (int32_t*)(ws + L.perm), *tl = (int32_t*)(ws + L.tiles);

@@ -574,6 +574,18 @@ class _HeldOwn:
         self.buf = None
 
 
+def _f8_launch(name: str, dev: torch.device, need: int, captured: bool, *args):
+    """The entry ``name`` with a workspace of ``need`` bytes. Where that has to be allocated, the call is first put
+    without one, which launches nothing: sizes and strides that it refuses must not take memory that is never given back."""
+    stream = _stream(dev)
+    if need > 0 and (captured or (ws := _WS.get((dev.index, stream))) is None or ws[0].numel() < need):
+        rc = getattr(_lib.lib(), name)(*args, None, 0, stream)
+        if rc != _lib.IMQ_ERR_SCRATCH:
+            raise _lib.ImqError(name, rc, _lib.lib().imq_strerror(rc).decode())
+    with (_HeldOwn if captured else _Held)(dev, need) as (ws, wsb):
+        call(name, *args, ws, wsb, stream)
+
+
 class _FastF8:
     """The native host path's fp8 and routing calls; each returns None for a call that is not a plain one."""
 
@@ -700,10 +712,9 @@ def linear_f8(x, qweight, scale, x_scale=None, out=None):
         raise ValueError("out must be a bf16 [M, N] tensor with unit column stride")
     y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     with torch.cuda.device(dev):
-        with (_HeldOwn if own else _Held)(dev, int(_lib.lib().imq_linear_f8_workspace_bytes(M, N, Kpad, code))) as (ws, wsb):
-            call("imq_linear_f8", _ptr(x), x.stride(0), code, M, K, _ptr(x_scale) if x_scale is not None else None, sm, sb,
-                 _ptr(qweight), qweight.stride(0), _ptr(scale), scale.stride(0), scale.stride(1), N, Kpad, _ptr(y),
-                 y.stride(0), ws, wsb, _stream(dev))
+        _f8_launch("imq_linear_f8", dev, int(_lib.lib().imq_linear_f8_workspace_bytes(M, N, Kpad, code)), own, _ptr(x),
+                   x.stride(0), code, M, K, _ptr(x_scale) if x_scale is not None else None, sm, sb, _ptr(qweight),
+                   qweight.stride(0), _ptr(scale), scale.stride(0), scale.stride(1), N, Kpad, _ptr(y), y.stride(0))
     return y
 
 
@@ -757,13 +768,15 @@ def moe_experts_f8(hidden, topk_idx, topk_w, gu, dn, workspace=None, *, check_id
     own = workspace is not None and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0 and \
         workspace.numel() * workspace.element_size() >= need
     out = torch.empty((T, H), dtype=torch.bfloat16, device=dev)
-    with torch.cuda.device(dev), (_HeldOwn if captured else _Held)(dev, 0 if own else need) as (ws, wsb):
+    args = (_ptr(x), x.stride(0), dtype_code(x.dtype), T, H, k, _ptr(idx),
+            _lib.IMQ_DT_I64 if idx.dtype == torch.int64 else _lib.IMQ_DT_I32, _ptr(w), dtype_code(w.dtype), E,
+            _ptr(gq), gq.stride(0), gq.stride(1), _ptr(gs), gs.stride(0), gs.stride(1), I, _ptr(dq), dq.stride(0),
+            dq.stride(1), _ptr(ds), ds.stride(0), ds.stride(1), _ptr(out), H)
+    with torch.cuda.device(dev):
         if own:
-            ws, wsb = _ptr(workspace), workspace.numel() * workspace.element_size()
-        call("imq_moe_experts_f8", _ptr(x), x.stride(0), dtype_code(x.dtype), T, H, k, _ptr(idx),
-             _lib.IMQ_DT_I64 if idx.dtype == torch.int64 else _lib.IMQ_DT_I32, _ptr(w), dtype_code(w.dtype), E,
-             _ptr(gq), gq.stride(0), gq.stride(1), _ptr(gs), gs.stride(0), gs.stride(1), I, _ptr(dq), dq.stride(0),
-             dq.stride(1), _ptr(ds), ds.stride(0), ds.stride(1), _ptr(out), H, ws, wsb, _stream(dev))
+            call("imq_moe_experts_f8", *args, _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(dev))
+        else:
+            _f8_launch("imq_moe_experts_f8", dev, need, captured, *args)
     return out
 
 

@@ -1,0 +1,87 @@
+"""What the fp8 operators do around a launch, without a device: refusals before any memory is taken, the stream that is asked
+about capture, outputs that lie over inputs, sizes at the ends of the C entry points."""
+import contextlib
+import ctypes
+
+import pytest
+import torch
+
+from infinitemodel_amd import _lib
+
+F8 = torch.float8_e4m3fn
+BF, F32 = _lib.IMQ_DT_BF16, _lib.IMQ_DT_FP32
+UNSUP, SCRATCH = _lib.IMQ_ERR_UNSUPPORTED, _lib.IMQ_ERR_SCRATCH
+P = ctypes.c_void_p(4096)          # never dereferenced: every call here is refused on the host
+TOP = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def L():
+    return _lib.lib()
+
+
+@pytest.fixture
+def host_ops(monkeypatch):
+    """ops on host tensors, the entries as they are (what gets past their checks fails for want of a device); a workspace
+    fails the test."""
+    from infinitemodel_amd import ops
+    monkeypatch.setattr(ops, "_check_dev", lambda *a: torch.device("cpu"))
+    monkeypatch.setattr(ops, "_stream", lambda dev: 0)
+    monkeypatch.setattr(ops, "_scratch", lambda *a: pytest.fail("took a workspace"))
+    monkeypatch.setattr(torch.cuda, "device", lambda dev: contextlib.nullcontext())
+    return ops
+
+
+def _experts(L, T, k, E, H, I, gsq=None, dsq=None, ws=P, wsb=1 << 62):
+    up = lambda n: -(-n // 128) * 128                                        # noqa: E731
+    gsq, dsq = up(H) if gsq is None else gsq, up(I) if dsq is None else dsq
+    return L.imq_moe_experts_f8(P, H, BF, T, H, k, P, _lib.IMQ_DT_I64, P, F32, E, P, 0, gsq, P, 0, 0, I, P, 0, dsq, P, 0, 0, P, H, ws,
+                                wsb, None)
+
+
+SIZES = [(131072, 8, 64, 7168, 2048), (262144, 8, 64, 8192, 2048), (1 << 24, 1, 4, 129, 128), (1 << 23, 2, 4, 128, 129), (4, 1, 4, 1 << 24, 256),
+         (4, 1, 4, 256, 1 << 24), (TOP, 1, 4, 1, 1), (1, TOP, 4, 1, 1), (1, 1, 4, TOP, 1), (1, 1, 4, 1, TOP), (TOP, TOP, 4, TOP, TOP),
+         (1 << 60, 1 << 60, 4, 1 << 60, 1 << 60), (3, 2, 4097, 128, 128), (1 << 24, 1, 4, 128, 128), (1 << 23, 1, 4, 128, 128)]
+
+
+@pytest.mark.parametrize("T,k,E,H,I", SIZES)
+def test_experts_sizes_that_are_refused_need_no_workspace(L, T, k, E, H, I):
+    """imq_moe_f8_workspace_bytes says -1 exactly where the entry refuses the sizes; it never overflows."""
+    need = L.imq_moe_f8_workspace_bytes(T, k, E, H, I)
+    rc = _experts(L, T, k, E, H, I, ws=None, wsb=0)
+    assert (need == -1) == (rc == UNSUP) and rc in (UNSUP, SCRATCH)
+    assert need == -1 or T * k * 4 * H < need < 2 ** 50
+
+
+def test_experts_strides_that_are_refused(L):
+    assert _experts(L, 3, 2, 4, 256, 128, ws=None, wsb=0) == SCRATCH
+    assert _experts(L, 3, 2, 4, 256, 128, gsq=1 << 26, ws=None, wsb=0) == UNSUP
+    assert _experts(L, 3, 2, 4, 256, 128, dsq=1 << 26, ws=None, wsb=0) == UNSUP
+
+
+def _refused(f):
+    with pytest.raises(_lib.ImqError) as e:
+        f()
+    assert e.value.status == UNSUP
+
+
+def test_refused_experts_take_no_memory(host_ops):
+    """Sizes past 32-bit offsets, and strides past them, are refused before a workspace is taken."""
+    stack = lambda E, N, K: torch.empty(E, N, -(-K // 128) * 128, dtype=F8)    # noqa: E731
+    T, k, H, I = 131072, 8, 7168, 2048
+    gu = (stack(1, 2 * I, H), torch.empty(1, 2 * I // 128, H // 128), H)
+    dn = (stack(1, H, I), torch.empty(1, H // 128, I // 128), I)
+    x = torch.empty(T, H, dtype=torch.bfloat16)
+    ids, w = torch.zeros(T, k, dtype=torch.int64), torch.ones(T, k)
+    for check in (True, False):
+        _refused(lambda: host_ops.moe_experts_f8(x, ids, w, gu, dn, check_ids=check))
+    far = torch.empty(128 << 24, dtype=torch.uint8).view(F8).as_strided((1, 128, 256), (0, 1 << 24, 1))   # never written
+    gu = (far, torch.empty(1, 2, 2), 256)
+    dn = (stack(1, 256, 64), torch.empty(1, 2, 1), 64)
+    _refused(lambda: host_ops.moe_experts_f8(x[:3, :256], ids[:3], w[:3], gu, dn, check_ids=False))
+
+
+def test_refused_linears_take_no_memory(host_ops):
+    far = torch.empty(2 << 24, dtype=torch.uint8).view(F8).as_strided((2, 512), (1 << 24, 1))
+    for M in (16, 40, 200):
+        _refused(lambda: host_ops.linear_f8(torch.empty(M, 64 << 7)[:, :512], far, torch.ones(1, 4)))
