@@ -147,11 +147,22 @@ def _first_moe(*a):
 _fast_linear, _fast_moe = _first_linear, _first_moe
 
 
+def _capturing(x) -> bool:
+    """Whether the current stream of x's device is being captured; torch's own query asks the current device's."""
+    index = x.get_device()
+    if index < 0:
+        return False
+    if index == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _check_expert_ids(idx: torch.Tensor, E: int) -> None:
     """Refuse routing ids outside [0, E), as the reference's eager experts loop does (its
     ``one_hot(num_classes=E)`` raises). One device-to-host read, so it is skipped while a HIP graph
     is being captured (the kernels then only keep out-of-range ids' loads in bounds)."""
-    if idx.numel() == 0 or (idx.is_cuda and torch.cuda.is_current_stream_capturing()):
+    if idx.numel() == 0 or _capturing(idx):
         return
     lo, hi = (int(v) for v in torch.aminmax(idx))
     if lo < 0 or hi >= E:
@@ -554,10 +565,6 @@ def moe_experts_w4(hidden, topk_idx, topk_w, gu, dn, group_size: int, workspace=
 # ---------------------------------------------------------------------------------------------
 # block-scaled fp8 (e4m3 codes, one fp32 scale per 128 columns of a row or 128 x 128 block of a weight)
 # ---------------------------------------------------------------------------------------------
-def _capturing(x) -> bool:
-    return x.is_cuda and torch.cuda.is_current_stream_capturing()
-
-
 class _HeldOwn:
     """A workspace for one call under graph capture: memory of the graph's own pool, so that graphs captured on one stream
     may be replayed on several without sharing it."""

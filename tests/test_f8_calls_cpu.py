@@ -85,3 +85,45 @@ def test_refused_linears_take_no_memory(host_ops):
     far = torch.empty(2 << 24, dtype=torch.uint8).view(F8).as_strided((2, 512), (1 << 24, 1))
     for M in (16, 40, 200):
         _refused(lambda: host_ops.linear_f8(torch.empty(M, 64 << 7)[:, :512], far, torch.ones(1, 4)))
+
+
+# ---- capture -------------------------------------------------------------------------------------
+class _OnDevice:
+    """As much of a tensor of device ``index`` as the questions about capture ask for."""
+    is_cuda = True
+
+    def __init__(self, index):
+        self.index, self.device = index, torch.device("cuda", index)
+
+    def get_device(self):
+        return self.index
+
+    def numel(self):
+        return 4
+
+
+@pytest.mark.parametrize("captured", [0, 1])
+@pytest.mark.parametrize("index", [0, 1])
+def test_capture_is_asked_of_the_tensor_s_device(monkeypatch, captured, index):
+    """With device 0 current, and the stream of one of two devices under capture: what counts is the stream of the device that the
+    call runs on, for the workspace and for the ids' check alike."""
+    from infinitemodel_amd import ops
+    now = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        old, now[0] = now[0], torch.device("cuda", d).index if isinstance(d, int) else torch.device(d).index
+        yield
+        now[0] = old
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] == captured)
+    monkeypatch.setattr(torch, "aminmax", lambda t: (0, 9))
+    x = _OnDevice(index)
+    assert ops._capturing(x) == (index == captured) and now[0] == 0
+    if index == captured:
+        ops._check_expert_ids(x, 4)                # a read would end the capture
+    else:
+        with pytest.raises(ValueError):
+            ops._check_expert_ids(x, 4)
+    assert not ops._capturing(torch.zeros(1))
