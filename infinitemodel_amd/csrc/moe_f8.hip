@@ -274,7 +274,9 @@ extern "C" int imq_moe_experts_f8(const void* hidden, int64_t h_row_stride, int 
     return IMQ_ERR_ALIGN;
   const int64_t lim = 0x7fffffff;
   const DevInfo dev = device_info();
-  if (!sizes_fit(T, top_k, E, H, I, dev) || 2 * I > lim / gu_q_row_stride || H > lim / dn_q_row_stride) return IMQ_ERR_UNSUPPORTED;
+  if (!sizes_fit(T, top_k, E, H, I, dev) || 2 * I > lim / gu_q_row_stride ||
+      (dn_q_row_stride > 0 && H > lim / dn_q_row_stride))      // one row of down needs no stride
+    return IMQ_ERR_UNSUPPORTED;
   const int64_t B = T * top_k;
   const Plan p = plan_of(T, top_k, E, H, I, dev);
   const Ws L = ws_of(p, T, top_k, E, H, I);

@@ -2,6 +2,9 @@
 about capture, outputs that lie over inputs, sizes at the ends of the C entry points."""
 import contextlib
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -127,3 +130,13 @@ def test_capture_is_asked_of_the_tensor_s_device(monkeypatch, captured, index):
         with pytest.raises(ValueError):
             ops._check_expert_ids(x, 4)
     assert not ops._capturing(torch.zeros(1))
+
+
+# ---- the ends of the C entries -------------------------------------------------------------------
+def test_one_row_of_down_without_a_stride():
+    """H = 1 takes any stride of down's one row, 0 as well; in a process of its own, as a division by it would end that."""
+    code = ("import ctypes, torch\nfrom infinitemodel_amd import _lib\nP = ctypes.c_void_p(4096)\n"
+            "f = lambda ds: _lib.lib().imq_moe_experts_f8(P, 1, 0, 3, 1, 2, P, 4, P, 2, 4, P, 0, 128, P, 0, 0, 128, P, 0, ds, P, 0, 0, "
+            "P, 1, None, 0, None)\nprint(f(0), f(128), f(-16))")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(__file__)))
+    assert r.returncode == 0 and r.stdout.split() == [str(SCRATCH), str(SCRATCH), str(_lib.IMQ_ERR_INVALID)], r
