@@ -141,7 +141,7 @@ extern "C" int imq_linear_f8(const void* x, int64_t x_row_stride, int x_dtype, i
       (given && (((uintptr_t)x & 15) || (x_row_stride & 15) || ((uintptr_t)x_scale & 3))) || ((uintptr_t)workspace & 15))
     return IMQ_ERR_ALIGN;
   const int64_t lim = 0x7fffffff, nb = K_pad / F8_BLOCK;
-  if (M > lim || N > lim || M > lim / 4 / nb || 257 * q_row_stride > lim || 257 * K_pad > lim || (given && 257 * x_row_stride > lim))
+  if (M > lim || N > lim || M > lim / 4 / nb || q_row_stride > lim / 257 || K_pad > lim / 257 || (given && x_row_stride > lim / 257))
     return IMQ_ERR_UNSUPPORTED;
   const DevInfo dev = device_info();
   const Plan p = plan_of(M, N, nb, given, dev);

@@ -140,3 +140,15 @@ def test_one_row_of_down_without_a_stride():
             "P, 1, None, 0, None)\nprint(f(0), f(128), f(-16))")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=os.path.dirname(os.path.dirname(__file__)))
     assert r.returncode == 0 and r.stdout.split() == [str(SCRATCH), str(SCRATCH), str(_lib.IMQ_ERR_INVALID)], r
+
+
+def test_linear_strides_whose_multiples_overflow(L):
+    """Row strides are held against the limit by division: 257 times this one is 256 in 64 bits."""
+    wraps = 0xff00ff00ff0100
+    assert wraps * 257 % 2 ** 64 == 256
+
+    def f(sx=512, dt=BF, sq=512, xs=None):
+        return L.imq_linear_f8(P, sx, dt, 40, 512, xs, 4, 1, P, sq, P, 4, 1, 300, 512, P, 300, None, 0, None)
+    assert f() == SCRATCH
+    assert f(sq=wraps) == UNSUP and f(sq=1 << 23) == UNSUP and f(sq=1 << 22) == SCRATCH
+    assert f(dt=_lib.IMQ_DT_F8, xs=P, sx=wraps) == UNSUP and f(dt=_lib.IMQ_DT_F8, xs=P, sx=1 << 23) == UNSUP
