@@ -275,7 +275,8 @@ int imq_pack_f8(const void* W, int64_t w_stride_e, int64_t w_row_stride, int w_d
  * 1.5e-5 of a sum of normal values, a hundredth of y's rounding).
  *   x: bf16 / fp16 / fp32 [M, K], quantized within the call as imq_quant_f8 does (K_pad - 128 < K <= K_pad); or,
  *     with x_dtype IMQ_DT_F8, e4m3 [M, K_pad] (K = K_pad) with x_scale[m, b] at m * xs_stride_m + b * xs_stride_b.
- *   qweight: e4m3 [N, K_pad], row stride in bytes; scale[r, b] at r * s_stride_r + b * s_stride_b.
+ *   qweight: e4m3 [N, K_pad], row stride in bytes; scale[r, b] at r * s_stride_r + b * s_stride_b. y shares no memory with any
+ *   of them: workgroups write it while others still read.
  *   workspace: device memory of imq_linear_f8_workspace_bytes(M, N, K_pad, x_dtype) bytes (the quantized rows,
  *     fp32 partials), 16-byte aligned, not initialised; IMQ_ERR_SCRATCH if it is less. Calls sharing one are
  *     ordered on one stream. Quantized rows and weights need 16-byte alignment, row strides included. */

@@ -647,6 +647,20 @@ def _f8_scale(s: torch.Tensor, shape, name: str) -> torch.Tensor:
     return s
 
 
+def _bytes_of(t: torch.Tensor):
+    """First byte and end of a non-empty tensor's memory."""
+    n = 1 + sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def _over(out: torch.Tensor, *inputs) -> bool:
+    """Whether ``out`` may share memory with an input that a launch still reads while it writes ``out``."""
+    if out.numel() == 0:
+        return False
+    a, b = _bytes_of(out)
+    return any(lo < b and a < hi for lo, hi in (_bytes_of(t) for t in inputs if t is not None and t.numel() > 0))
+
+
 def quant_f8(x):
     """Rows to block-scaled e4m3: ``(q float8_e4m3fn [M, K_pad], scale fp32 [M, K_pad / 128])``, K_pad = K rounded up to
     128 with zero codes. A block's scale is max(amax|x| / 448, 2^-100), its codes x / scale rounded once to nearest
@@ -694,8 +708,8 @@ def linear_f8(x, qweight, scale, x_scale=None, out=None):
     """``y[M, N] bf16 = x W^T`` of block-scaled e4m3 operands: the products of a block of 128 columns are summed and
     taken times both scales in fp32. ``x`` [.., K] bf16 / fp16 / fp32 is quantized within the call as ``quant_f8`` does
     (K_pad - 128 < K <= K_pad), or handed over quantized (e4m3 [M, K_pad], ``x_scale`` [M, K_pad / 128]). ``qweight``
-    e4m3 [N, K_pad], ``scale`` fp32 [ceil(N / 128), K_pad / 128], as ``pack_f8`` gives them. No counterpart in the
-    reference."""
+    e4m3 [N, K_pad], ``scale`` fp32 [ceil(N / 128), K_pad / 128], as ``pack_f8`` gives them. ``out``: where the result
+    goes, a bf16 [M, N] tensor; one that lies over an input gets it by a copy at the end. No counterpart in the reference."""
     own = _capturing(x)
     if out is None and not own and (y := _fast_f8.linear_f8(x, qweight, scale, x_scale)) is not None:
         return y
@@ -717,12 +731,15 @@ def linear_f8(x, qweight, scale, x_scale=None, out=None):
     if out is not None and (tuple(out.shape) != (M, N) or out.dtype != torch.bfloat16 or out.stride(1) != 1 or
                             (M > 1 and out.stride(0) < N) or out.device != dev):
         raise ValueError("out must be a bf16 [M, N] tensor with unit column stride")
-    y = out if out is not None else torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    y = out if out is not None and not _over(out, x, qweight, scale, x_scale) else \
+        torch.empty((M, N), dtype=torch.bfloat16, device=dev)
     with torch.cuda.device(dev):
         _f8_launch("imq_linear_f8", dev, int(_lib.lib().imq_linear_f8_workspace_bytes(M, N, Kpad, code)), own, _ptr(x),
                    x.stride(0), code, M, K, _ptr(x_scale) if x_scale is not None else None, sm, sb, _ptr(qweight),
                    qweight.stride(0), _ptr(scale), scale.stride(0), scale.stride(1), N, Kpad, _ptr(y), y.stride(0))
-    return y
+        if out is not None and y is not out:
+            out.copy_(y)
+    return y if out is None else out
 
 
 def moe_f8_workspace_bytes(T: int, top_k: int, E: int, H: int, I: int) -> int:

@@ -132,6 +132,34 @@ def test_capture_is_asked_of_the_tensor_s_device(monkeypatch, captured, index):
     assert not ops._capturing(torch.zeros(1))
 
 
+# ---- out over an input ---------------------------------------------------------------------------
+def test_out_over_an_input_is_not_what_the_launch_writes(host_ops, monkeypatch):
+    """Where out shares memory with x, the weights or a scale, the launch gets a tensor of its own and out a copy of it; elsewhere,
+    also right beside an input, out itself."""
+    seen = []
+
+    def launch(name, dev, need, captured, *a):
+        seen.append(a[-2])                         # y: filled as a kernel would
+        ctypes.memset(a[-2], 0x40, 2 * 256)
+    monkeypatch.setattr(host_ops, "_f8_launch", launch)
+    buf = torch.zeros(3, 256, dtype=torch.bfloat16)
+    raw = torch.zeros(1 << 16, dtype=torch.uint8)
+    q, s = raw.view(F8).view(256, 256), torch.ones(2, 512)[:, ::256]
+    xq, xs = torch.zeros(1, 256).to(F8), torch.ones(1, 512)[:, ::256]
+
+    def over(t, at):                               # a [1, 256] bf16 view of t's memory from byte `at`
+        return torch.empty(0, dtype=torch.bfloat16).set_(t.untyped_storage(), at // 2, (1, 256))
+    x = buf[:1]
+    for call, out, own in ((lambda o: host_ops.linear_f8(x, q, s, out=o), buf[1:2], False),
+                           (lambda o: host_ops.linear_f8(x, q, s, out=o), buf[:1], True),
+                           (lambda o: host_ops.linear_f8(x, q, s, out=o), over(raw, 1000), True),
+                           (lambda o: host_ops.linear_f8(x, q, s, out=o), over(s, 600), True),
+                           (lambda o: host_ops.linear_f8(xq, q, s, x_scale=xs, out=o), over(xs, 600), True)):
+        y = call(out)
+        assert (seen[-1] != out.data_ptr()) == own and y.data_ptr() == out.data_ptr()
+        assert bool((out.view(torch.uint8) == 0x40).all())
+
+
 # ---- the ends of the C entries -------------------------------------------------------------------
 def test_one_row_of_down_without_a_stride():
     """H = 1 takes any stride of down's one row, 0 as well; in a process of its own, as a division by it would end that."""

@@ -22,3 +22,20 @@ def test_refused_sizes_take_no_workspace(dev, monkeypatch):
                 ops.moe_experts_f8(x, ids, w, gu, dn, check_ids=check)
             assert e.value.status == _lib.IMQ_ERR_UNSUPPORTED
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 40])
+def test_out_over_x(dev, M):
+    """A result that goes where its input is (or a row further) is that of a call with an output of its own."""
+    import torch
+    from infinitemodel_amd import ops
+    K = 2048
+    W = torch.randn(K, K, generator=torch.Generator().manual_seed(M)) * 0.02
+    q, s, _ = ops.pack_f8(W.to(dev))
+    x = torch.randn(M + 1, K, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16).to(dev)
+    want = ops.linear_f8(x[:M], q, s)
+    for row in (0, 1):
+        buf = x.clone()
+        y = ops.linear_f8(buf[:M], q, s, out=buf[row:row + M])
+        assert y.data_ptr() == buf[row].data_ptr() and torch.equal(y, want)
+        assert torch.equal(buf[M if row == 0 else 0], x[M if row == 0 else 0])
