@@ -57,10 +57,12 @@ def dequantize(codes, scale, rows=1):
     return v * np.repeat(s, BLOCK, axis=1)
 
 
-def sum_slack(K):
-    """Relative to the sum of the magnitudes: K products summed in fp32 in any order, each addition off by at most a
-    whole step of 2^-23, and as many roundings of scales and blocks as there are."""
-    return (K + 3 * blocks(K) + 8) * 2.0 ** -23
+def sum_slack(K, rows=1):
+    """Relative to the sum of the magnitudes: `rows` sums of K products each, taken as one. The products of a block of 128 columns
+    are exact and summed first, in any order, each addition off by at most a whole step of 2^-23 (an instruction may cut);
+    then every block is taken times one factor, which is rounded, and joined by an fma, the waves' sums and those of K
+    ranges by additions, all off by half a step: at most three roundings a block, and four besides."""
+    return (2 * min(K, BLOCK) + 3 * rows * blocks(K) + 4) * 2.0 ** -24
 
 
 def cut_slack(xv, wv):
@@ -111,7 +113,7 @@ def experts(xv, ids, w, gu, dn, H, I):
         lo, hi = (values_of(codes_of(np.clip(a + d, 0.0, TOP))) for d in (-move, move))
         width = np.maximum(np.abs(hi * sv - np.abs(hv)), np.abs(lo * sv - np.abs(hv))) + np.maximum(hi, np.abs(hv) / sv) * es
         y = hv @ wd.T
-        ey = width @ np.abs(wd).T + sum_slack(hv.shape[1]) * ((np.abs(hv) + width) @ np.abs(wd).T) + cut_slack(np.abs(hv) + width, wd)
+        ey = width @ np.abs(wd).T + sum_slack(hv.shape[1], k) * ((np.abs(hv) + width) @ np.abs(wd).T) + cut_slack(np.abs(hv) + width, wd)
         c = w[t, j].astype(np.float64)[:, None]
         np.add.at(out, t, c * y)
         np.add.at(tol, t, np.abs(c) * ey + k * 2.0 ** -23 * np.abs(c * y))
