@@ -397,6 +397,12 @@ int imq_gptq_int2_solve(float* W, int64_t ldw, int64_t out, int64_t in_f, const 
  *     IMQ_PLAN_GEMM_RBM   register-B GEMM at any tile height (M > 64, bf16 / fp16 scale and zero
  *                         alike; the format by q_row_stride, dense rows): p1 32-row blocks (int4 and int2 in
  *                         rows may run taller ones where the tiles outnumber the CUs), p2 K splits
+ *     IMQ_PLAN_LINEAR_F8  imq_linear_f8 (s_dtype: x's, IMQ_DT_F8 for rows handed over quantized): p1 weight rows a tile, p2
+ *                         activation rows, p3 K ranges; or, of the few-row kernel, p1 0, p2 waves, p3 0 where quantized
+ *                         rows are read beside the weights, 1 where rows are quantized inside, 2 where quantized ones are
+ *                         copied to LDS
+ *     IMQ_PLAN_MOE_F8     imq_moe_experts_f8 (in: T, H, top_k, I, E in the first five places): p1 routed rows a tile; or, of the direct
+ *                         form, p1 0, p2 waves of gate_up, p3 of down
  * Returns IMQ_OK, or IMQ_ERR_INVALID for an unknown kind or a null pointer. */
 #define IMQ_PLAN_W4_LINE 1
 #define IMQ_PLAN_W4_KSPLIT 2
@@ -409,6 +415,8 @@ int imq_gptq_int2_solve(float* W, int64_t ldw, int64_t out, int64_t in_f, const 
 #define IMQ_PLAN_GEMM_RB 9
 #define IMQ_PLAN_GEMM_WK 10
 #define IMQ_PLAN_GEMM_RBM 11
+#define IMQ_PLAN_LINEAR_F8 12
+#define IMQ_PLAN_MOE_F8 13
 int imq_launch_plan(int kind, const int64_t* in, int64_t* out);
 
 #ifdef __cplusplus

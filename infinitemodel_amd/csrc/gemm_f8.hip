@@ -115,6 +115,24 @@ bool float_type(int dt) { return dt == IMQ_DT_BF16 || dt == IMQ_DT_FP16 || dt ==
 
 }  // namespace
 
+namespace imq {
+
+// imq_launch_plan's answer for imq_linear_f8.
+void linear_f8_plan_query(int64_t M, int64_t N, int64_t K_pad, bool given, int cus, int max_lds, int64_t* out) {
+  const int64_t nb = K_pad / F8_BLOCK;
+  const Plan p = plan_of(M, N, nb, given, DevInfo{cus, max_lds});
+  const TileCost& t = kTiles[p.tile];
+  constexpr int lds[] = {f8_tile_lds(256, 256, 8, 2, 0), f8_tile_lds(128, 128, 4, 2, 0), f8_tile_lds(128, 64, 4, 3, 0),
+                         f8_tile_lds(64, 64, 4, 4, 0), f8_tile_lds(64, 32, 2, 5, 0)};
+  out[0] = 1;
+  out[1] = p.waves > 0 ? 0 : t.bn;
+  out[2] = p.waves > 0 ? p.waves : t.bm;
+  out[3] = p.waves > 0 ? (p.inside ? 1 : p.copy ? 2 : 0) : p.splits;
+  out[4] = p.waves > 0 ? f8_gemv_lds(p.waves, 0, !p.inside && !p.copy, M, nb) : lds[p.tile];
+}
+
+}  // namespace imq
+
 extern "C" int64_t imq_linear_f8_workspace_bytes(int64_t M, int64_t N, int64_t K_pad, int x_dtype) {
   if (M < 0 || N < 0 || K_pad < 0 || K_pad % F8_BLOCK || !(float_type(x_dtype) || x_dtype == IMQ_DT_F8)) return -1;
   if (M == 0 || N == 0 || K_pad == 0) return 0;

@@ -39,6 +39,8 @@ void gemm_plan_query(int64_t M, int64_t N, int64_t K, int cus, int64_t* out);
 void wk_plan_query(int bits, int64_t M, int64_t N, int64_t K, int64_t G, int cus, int max_lds, int64_t* out);
 void rbm_plan_query(int bits, int64_t M, int64_t N, int64_t K, int64_t G, int cus, int64_t* out);
 void rb_plan_query(int bits, int64_t M, int64_t N, int64_t K, int64_t G, int cus, int64_t* out);
+void linear_f8_plan_query(int64_t M, int64_t N, int64_t K_pad, bool given, int cus, int max_lds, int64_t* out);
+void moe_f8_plan_query(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int cus, int max_lds, int64_t* out);
 int gemm_wkd(int bits, const uint16_t* x, int64_t sxm, int64_t M, int64_t K, const uint8_t* q, int64_t sqn,
              const void* sc, int64_t ssn, int64_t ssg, int sdt, const void* zr, int64_t szn, int64_t szg, int zdt,
              int64_t N, int64_t G, uint16_t* y, int64_t sym, hipStream_t st);
@@ -135,6 +137,16 @@ extern "C" int imq_launch_plan(int kind, const int64_t* in, int64_t* out) {
       return IMQ_OK;
     }
     imq::wk_plan_query((int)bits, M, N, K, G, cus, (int)in[8], out);
+    return IMQ_OK;
+  }
+  if (kind == IMQ_PLAN_LINEAR_F8) {
+    const int64_t lim = 0x7fffffff;
+    if (cus > 0 && M > 0 && N > 0 && K > 0 && K % 128 == 0 && M <= lim && N <= lim && K <= lim)
+      imq::linear_f8_plan_query(M, N, K, in[7] == IMQ_DT_F8, cus, (int)in[8], out);
+    return IMQ_OK;
+  }
+  if (kind == IMQ_PLAN_MOE_F8) {
+    if (cus > 0 && M > 0 && K > 0 && G > 0 && N > 0 && in[4] > 0) imq::moe_f8_plan_query(M, G, in[4], K, N, cus, (int)in[8], out);
     return IMQ_OK;
   }
   if (in[7] != IMQ_DT_BF16 && in[7] != IMQ_DT_FP16 && in[7] != IMQ_DT_FP32) return IMQ_ERR_INVALID;

@@ -246,6 +246,24 @@ bool sizes_fit(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, const DevI
 
 }  // namespace
 
+namespace imq {
+
+// imq_launch_plan's answer for imq_moe_experts_f8 (LDS: gate_up's).
+void moe_f8_plan_query(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, int cus, int max_lds, int64_t* out) {
+  const DevInfo dev{cus, max_lds};
+  if (!sizes_fit(T, k, E, H, I, dev)) return;
+  const Plan p = plan_of(T, k, E, H, I, dev);
+  out[0] = 1;
+  out[1] = p.direct ? 0 : p.bm;
+  out[2] = p.direct ? p.wg : 0;
+  out[3] = p.direct ? p.wd : 0;
+  out[4] = p.direct ? f8_gemv_lds(p.wg, 1, false, 1, imq_cdiv(H, F8_BLOCK))
+           : p.bm == 192 ? f8_tile_lds(256, 192, 8, 2, 1) : p.bm == 128 ? f8_tile_lds(256, 128, 8, 2, 1)
+           : p.bm == 64 ? f8_tile_lds(256, 64, 4, 3, 1) : f8_tile_lds(256, 32, 4, 4, 1);
+}
+
+}  // namespace imq
+
 extern "C" int64_t imq_moe_f8_workspace_bytes(int64_t T, int64_t top_k, int64_t E, int64_t H, int64_t I) {
   if (T < 0 || top_k < 1 || E < 1 || H < 1 || I < 1) return -1;
   if (T == 0) return 0;
