@@ -180,8 +180,10 @@ Plan plan_of(int64_t T, int64_t k, int64_t E, int64_t H, int64_t I, const DevInf
   const double w = 3.0 * H * I / 1e6, hit = (double)E * (1.0 - pow(1.0 - (double)(k < E ? k : E) / E, (double)T));
   p.direct = B <= 64 && B * w / 5.6 + 6.0 <= hit * w / 5.2 + 14.0 && f8_gemv_lds(p.wg, 1, false, 1, hb) <= d.max_lds && f8_gemv_lds(p.wd, 2, false, k, ib) <= d.max_lds &&
              (k * ib + 1) * 128 < 0x7fffffff;
-  // Rows a tile by the mean rows an expert: short experts leave a tall tile empty, tall tiles read the weights less often (250
-  // rows: 192 259 us, 128 282; 256 of smaller experts 283 and 279; 175: 122 and 96; 128: 212 and 196).
+  // Rows a tile by the mean rows an expert: short experts leave a tall tile empty, tall tiles read the weights less often. us in
+  // tiles of 192 and of 128 rows: 200 rows an expert, 64 experts of 2048 x 1408 362 and 336; 250 rows, 64 of 2048 x 1024 301 and
+  // 288, but 8 of 4096 x 1792 134 and 158; 256 rows, 64 of 2048 x 768 243 and 240, 16 of 2048 x 1024 93 and 115; 512 rows, 64
+  // of 2048 x 1024 525 and 539. Between 200 and 256 the border follows the larger differences.
   p.bm = per > 224 ? 192 : per > 64 ? 128 : per > 24 ? 64 : 32;
   return p;
 }

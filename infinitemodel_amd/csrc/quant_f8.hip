@@ -7,8 +7,8 @@
 namespace {
 
 // 16 lanes of 8 columns hold a block; a workgroup takes 16 U consecutive blocks in row-major order, all of its loads
-// out before the first is used. HBM-bound: two thirds of the bytes are read, one third written (8192 x 8192 bf16: 41 us,
-// 4.9 TB/s; a plain device copy 5.1). The codes are stored as usual: the product reads them next.
+// out before the first is used. HBM-bound: two thirds of the bytes are read, one third written (8192 x 8192 bf16: 43.8 us,
+// 4.6 TB/s; a device copy of torch's 5.5). The codes are stored as usual: the product reads them next.
 template <int DT, int U>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict__ x, int64_t sx, uint32_t blocks,
                                                          int64_t K, FastDiv nbd, uint8_t* __restrict__ q, int64_t sq,
@@ -42,8 +42,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void* __restrict_
 
 // A workgroup per 128 x 128 block: 16 lanes of 8 columns per row, 16 rows at a time, the block's 64 values a
 // thread held in registers between the maximum and the division. HBM-bound, with the quotients' arithmetic (about 12
-// operations a value) at two thirds of that time: 28672 x 4096 bf16 68 us, 5.2 TB/s. The codes of a load-time
-// conversion are not read soon, so they are stored past the caches (71 us without).
+// operations a value) at two thirds of that time: 28672 x 4096 bf16 65.6 us, 5.4 TB/s. The codes of a load-time
+// conversion are not read soon, so they are stored past the caches (69.7 us without).
 template <int DT>
 __global__ __launch_bounds__(256) void pack_f8_kernel(const void* __restrict__ W, int64_t swe, int64_t sw, int64_t N,
                                                       int64_t K, int64_t mb, int64_t nb, uint8_t* __restrict__ q,
@@ -99,7 +99,8 @@ int quant_rows_f8(const void* x, int64_t sx, int dt, int64_t M, int64_t K, uint8
   const int64_t nb = imq_cdiv(K, F8_BLOCK);
   if (M > 0x7fffffff / nb) return IMQ_ERR_UNSUPPORTED;
   const int64_t blocks = M * nb;
-  // two blocks a lane group where that still leaves eight workgroups a CU (2048 x 14336: 18.6 us, one 19.4, four 20.5)
+  // two blocks a lane group where that still leaves eight workgroups a CU (8192 x 8192: 43.8 us, one
+  // 45.3, four 44.7; 2048 x 14336: 19.5, 19.5, 20.8)
   const int U = blocks >= 32 * 8 * (int64_t)device_info().cus ? 2 : 1;
   const dim3 grid((unsigned)imq_cdiv(blocks, 16 * U));
   const FastDiv nbd = fast_div((uint32_t)nb);
